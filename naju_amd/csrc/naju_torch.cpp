@@ -51,6 +51,16 @@ void check_loss(int rc) { TORCH_CHECK(rc == NAJU_OK, "naju error ", rc, ": ", na
 bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool records(const optional<Tensor>& t) { return t && records(*t); }
 
+// A forward-mode tangent of an operand is refused, whether a graph is recorded
+// or not: the kernels know nothing of it, and a result without a tangent counts
+// as constant.
+void no_tangent(const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), "naju: forward-mode derivatives (jvp) are not served");
+}
+void no_tangent(const optional<Tensor>& t) {
+  if (t) no_tangent(*t);
+}
+
 // A second derivative is refused, not taken as zero.
 void once_differentiable(const variable_list& grads) {
   if (!at::GradMode::is_enabled()) return;
@@ -183,11 +193,13 @@ struct LayerNormFork : torch::autograd::Function<LayerNormFork> {
 };
 
 Tensor layer_norm(const Tensor& x, const optional<Tensor>& w, const optional<Tensor>& b, double eps, int64_t out) {
+  no_tangent(x), no_tangent(w), no_tangent(b);
   if (!records(x) && !records(w) && !records(b)) return norm_forward(nullptr, x, w, b, eps, out);
   return LayerNorm::apply(x, w, b, eps, out);
 }
 std::tuple<Tensor, Tensor> layer_norm_fork(const Tensor& x, const optional<Tensor>& w, const optional<Tensor>& b,
                                            double eps, int64_t out) {
+  no_tangent(x), no_tangent(w), no_tangent(b);
   auto r = LayerNormFork::apply(x, w, b, eps, out);
   return {r[0], r[1]};
 }
@@ -257,6 +269,7 @@ struct Gated : torch::autograd::Function<Gated> {
 };
 
 Tensor gated_linear(const Tensor& x, const Tensor& wg, const Tensor& wu, const optional<Tensor>& pair, int64_t act) {
+  no_tangent(x), no_tangent(wg), no_tangent(wu);
   if (!records(x) && !records(wg) && !records(wu)) return Gated::forward(nullptr, x, wg, wu, pair, act);
   return Gated::apply(x, wg, wu, pair, act);
 }
@@ -327,6 +340,7 @@ struct LinearXent : torch::autograd::Function<LinearXent> {
 
 Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& target, const optional<Tensor>& w16,
                             int64_t ignore, int64_t reduction) {
+  no_tangent(x), no_tangent(weight);
   if (!records(x) && !records(weight)) return LinearXent::forward(nullptr, x, weight, target, w16, ignore, reduction);
   return LinearXent::apply(x, weight, target, w16, ignore, reduction);
 }
