@@ -61,11 +61,33 @@ void no_tangent(const optional<Tensor>& t) {
   if (t) no_tangent(*t);
 }
 
-// A second derivative is refused, not taken as zero.
-void once_differentiable(const variable_list& grads) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor& g : grads)
-    TORCH_CHECK(!g.defined() || !g.requires_grad(), "naju: this backward is not differentiable itself");
+// What a backward that may itself be differentiated (create_graph) hands its
+// gradients on with: it leads to all that they depend on, and raises when a
+// second derivative is taken through it, whichever way and for whichever of
+// them. Without it their dependence would count as zero.
+struct Refusal : torch::autograd::Node {
+  explicit Refusal(const char* of) : of_(of) {}
+  variable_list apply(variable_list&&) override {
+    TORCH_CHECK(false, "naju: ", of_, " has no second derivative (its gradient does not require grad further)");
+  }
+  std::string name() const override { return "NajuSecondDerivative"; }
+  const char* of_;
+};
+variable_list once_differentiable(const char* of, const variable_list& incoming, variable_list grads) {
+  const auto self = torch::autograd::get_current_node();
+  if (!at::GradMode::is_enabled() || !self) return grads;
+  // the way to the operator's own inputs, and to what the incoming gradients came from
+  torch::autograd::edge_list next = self->next_edges();
+  for (const Tensor& g : incoming)
+    if (g.defined() && g.requires_grad()) next.push_back(torch::autograd::impl::gradient_edge(g));
+  const std::shared_ptr<Refusal> node(new Refusal(of), torch::autograd::deleteNode);
+  node->set_next_edges(std::move(next));
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach();
+    torch::autograd::create_gradient_edge(g, node);
+  }
+  return grads;
 }
 
 // t [..., d] as [rows, d] with d fastest and rows at least d apart: a view where there is one.
@@ -171,8 +193,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return norm_forward(ctx, x, w, b, eps, out);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once_differentiable(g);
-    return norm_backward(ctx, g[0], Tensor());
+    return once_differentiable("layer_norm", g, norm_backward(ctx, g[0], Tensor()));
   }
 };
 
@@ -185,9 +206,8 @@ struct LayerNormFork : torch::autograd::Function<LayerNormFork> {
     return {x.view(x.sizes()), y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once_differentiable(g);
-    if (g[1].defined()) return norm_backward(ctx, g[1], g[0]);
-    // only the stream was used
+    if (g[1].defined()) return once_differentiable("layer_norm", g, norm_backward(ctx, g[1], g[0]));
+    // only the stream was used: its gradient as it is
     return {g[0], Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -237,7 +257,6 @@ struct Gated : torch::autograd::Function<Gated> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_differentiable(grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor &m = saved[0], &gw = saved[1], &uw = saved[2];
     const auto type = m.scalar_type();
@@ -263,8 +282,8 @@ struct Gated : torch::autograd::Function<Gated> {
                                  (int)data.at("act").toInt(), code_of(type), code_of(w_type), ws.data_ptr(), bytes,
                                  stream_of(m)));
     }
-    return {need_x ? dx.view(shape) : dx, need_w ? as(dg, g_type) : dg, need_w ? as(du, u_type) : du, Tensor(),
-            Tensor()};
+    return once_differentiable("gated_linear", grads, {need_x ? dx.view(shape) : dx, need_w ? as(dg, g_type) : dg,
+                                                       need_w ? as(du, u_type) : du, Tensor(), Tensor()});
   }
 };
 
@@ -310,7 +329,6 @@ struct LinearXent : torch::autograd::Function<LinearXent> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once_differentiable(grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor &m = saved[0], &w = saved[1], &target = saved[2], &lse = saved[3], &scale = saved[4];
     const auto type = m.scalar_type();
@@ -334,7 +352,9 @@ struct LinearXent : torch::autograd::Function<LinearXent> {
                                       (const float*)ptr(scale), (const float*)dloss.data_ptr(), !scale.defined(),
                                       ptr(dx), ptr(dw), code_of(dw_type), ws.data_ptr(), bytes, stream_of(m)));
     }
-    return {need_x ? dx.view(shape) : dx, need_w ? as(dw, w_type) : dw, Tensor(), Tensor(), Tensor(), Tensor()};
+    return once_differentiable("linear_cross_entropy", grads, {need_x ? dx.view(shape) : dx,
+                                                               need_w ? as(dw, w_type) : dw, Tensor(), Tensor(),
+                                                               Tensor(), Tensor()});
   }
 };
 

@@ -44,7 +44,8 @@ class _ToTied(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dw):
-        if dw.dtype != torch.float32:
+        # (one with a graph of its own, create_graph, keeps it only on autograd's way)
+        if dw.dtype != torch.float32 or dw.requires_grad:
             return dw, None
         ctx.tied.put(dw)
         return None, None
