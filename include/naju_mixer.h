@@ -194,8 +194,9 @@ int naju_embedding_bwd_add(const int64_t* sorted_ids, const int64_t* order, cons
  * x [n_rows, d] with x_ld >= d elements between rows and d fastest, at any
  * element alignment; y [n_rows, d] contiguous; w and b [d] float32 (each
  * nullable: 1 and 0); mean and rstd [n_rows] float32 for the backward (both
- * or neither). x, y in F32, BF16 or F16 each; float32 arithmetic. No
- * reference counterpart (the reference's blocks use RMSNorm). */
+ * or neither). x, y in F32, BF16 or F16 each; float32 arithmetic. n_rows up to
+ * 2^31 - 1, d to 2^30. No reference counterpart (the reference's blocks use
+ * RMSNorm). */
 int naju_layernorm_fwd(const void* x, int64_t x_ld, const float* w, const float* b, float eps, void* y, float* mean,
                        float* rstd, int64_t n_rows, int64_t d, int x_dtype, int y_dtype, void* stream);
 

@@ -389,36 +389,39 @@ __global__ __launch_bounds__(64 * kWaves) void norm_cols_any_kernel(const NormAr
 }
 
 // dw[c], db[c] = the sums over n rows of part [n][2][d], in a fixed order: 32
-// columns a workgroup, each of 32 groups of lanes adds every 32nd row.
+// columns a workgroup at a time, each of 32 groups of lanes adds every 32nd row.
 __global__ __launch_bounds__(1024) void norm_fold_kernel(const float* __restrict__ part, int n, int64_t d,
                                                          float* __restrict__ dw, float* __restrict__ db) {
   __shared__ float s[32][33];
   const int col = threadIdx.x & 31, q = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + col;
-  float acc = 0.f;
-  if (c < 2 * d) {
-    constexpr int kU = 8;  // rows loaded before the first is added
-    int i = q;
-    for (; i + (kU - 1) * 32 < n; i += kU * 32) {
-      float v[kU];
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < 2 * d; c0 += (int64_t)gridDim.x * 32) {
+    const int64_t c = c0 + col;
+    float acc = 0.f;
+    if (c < 2 * d) {
+      constexpr int kU = 8;  // rows loaded before the first is added
+      int i = q;
+      for (; i + (kU - 1) * 32 < n; i += kU * 32) {
+        float v[kU];
 #pragma unroll
-      for (int u = 0; u < kU; ++u) v[u] = part[(int64_t)(i + u * 32) * 2 * d + c];
+        for (int u = 0; u < kU; ++u) v[u] = part[(int64_t)(i + u * 32) * 2 * d + c];
 #pragma unroll
-      for (int u = 0; u < kU; ++u) acc += v[u];
+        for (int u = 0; u < kU; ++u) acc += v[u];
+      }
+      for (; i < n; i += 32) acc += part[(int64_t)i * 2 * d + c];
     }
-    for (; i < n; i += 32) acc += part[(int64_t)i * 2 * d + c];
-  }
-  s[q][col] = acc;
-  __syncthreads();
-  if (q == 0 && c < 2 * d) {
-    float t = 0.f;
+    s[q][col] = acc;
+    __syncthreads();
+    if (q == 0 && c < 2 * d) {
+      float t = 0.f;
 #pragma unroll
-    for (int w = 0; w < 32; ++w) t += s[w][col];
-    if (c < d) {
-      if (dw) dw[c] = t;
-    } else if (db) {
-      db[c - d] = t;
+      for (int w = 0; w < 32; ++w) t += s[w][col];
+      if (c < d) {
+        if (dw) dw[c] = t;
+      } else if (db) {
+        db[c - d] = t;
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -531,7 +534,11 @@ void bwd_launch(const NormArgs& g, float* dw, float* db, hipStream_t st) {
     norm_bwd_kernel<TX, TY, kWaves, 4><<<grid, blk, 0, st>>>(g);
   else
     norm_bwd_kernel<TX, TY, kWaves, 8><<<grid, blk, 0, st>>>(g);
-  if (g.part) norm_fold_kernel<<<dim3((unsigned)((2 * g.d + 31) / 32)), 1024, 0, st>>>(g.part, (int)n, g.d, dw, db);
+  if (g.part) {
+    // (a launch has fewer than 2^32 threads: wider rows take turns)
+    const int64_t folds = (2 * g.d + 31) / 32, most = 1 << 20;
+    norm_fold_kernel<<<dim3((unsigned)(folds < most ? folds : most)), 1024, 0, st>>>(g.part, (int)n, g.d, dw, db);
+  }
 }
 
 template <typename TX>
