@@ -290,31 +290,37 @@ __global__ __launch_bounds__(64 * kWaves) void norm_bwd_kernel(const NormArgs g)
 }
 
 // Rows of any other width (below kV, or more than a workgroup holds), a
-// workgroup each, read again for every pass.
+// workgroup each, read again for every pass. A lane's share of a wide row has no
+// bound, so what it adds up over it is held in 64 bits: float32 sums of squares
+// over 2^26 columns left rstd off by 3e-5.
 template <typename TX, typename TY>
 __global__ __launch_bounds__(64 * kWaves) void norm_fwd_any_kernel(const NormArgs g) {
   __shared__ float2 s_red[2][4];
   const int64_t r = blockIdx.x;
   const TX* row = (const TX*)g.x + r * g.x_ld;
-  float s = 0.f;
+  double s = 0.0;
   for (int64_t c = threadIdx.x * kV; c < g.d; c += 64 * kWaves * kV) {
     float v[kV];
     load8(row, c, g.d, v);
+    float p = 0.f;
 #pragma unroll
-    for (int e = 0; e < kV; ++e) s += v[e];
+    for (int e = 0; e < kV; ++e) p += v[e];
+    s += (double)p;
   }
-  const float mean = row_sum<kWaves>(s, s_red, 0) / (float)g.d;
-  s = 0.f;
+  const float mean = row_sum<kWaves>((float)s, s_red, 0) / (float)g.d;
+  s = 0.0;
   for (int64_t c = threadIdx.x * kV; c < g.d; c += 64 * kWaves * kV) {
     float v[kV];
     load8(row, c, g.d, v);
+    float p = 0.f;
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
       const float u = c + e < g.d ? v[e] - mean : 0.f;
-      s = fmaf(u, u, s);
+      p = fmaf(u, u, p);
     }
+    s += (double)p;
   }
-  const float rstd = 1.f / sqrtf(row_sum<kWaves>(s, s_red, 1) / (float)g.d + g.eps);
+  const float rstd = 1.f / sqrtf(row_sum<kWaves>((float)s, s_red, 1) / (float)g.d + g.eps);
   for (int64_t c = threadIdx.x * kV; c < g.d; c += 64 * kWaves * kV) {
     float v[kV], w[kV], b[kV];
     load8(row, c, g.d, v);
@@ -342,6 +348,7 @@ __global__ __launch_bounds__(64 * kWaves) void norm_dx_any_kernel(const NormArgs
   const float mean = g.mean[r], rstd = g.rstd[r];
   const TX* x = (const TX*)g.x + r * g.x_ld;
   const TY* dy = (const TY*)g.dy + r * g.dy_ld;
+  double t1 = 0.0, t2 = 0.0;
   float s1 = 0.f, s2 = 0.f;
   for (int pass = 0; pass < 2; ++pass) {
     for (int64_t c = threadIdx.x * kV; c < g.d; c += 64 * kWaves * kV) {
@@ -350,53 +357,90 @@ __global__ __launch_bounds__(64 * kWaves) void norm_dx_any_kernel(const NormArgs
       load8(dy, c, g.d, gv);
       if (g.w) load8(g.w, c, g.d, w);
       if (pass && g.dres) load8((const TX*)g.dres + r * g.d, c, g.d, res);
+      float p1 = 0.f, p2 = 0.f;
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
         const float xh = (xv[e] - mean) * rstd;
         if (g.w) gv[e] *= w[e];
         if (pass == 0) {
-          s1 += gv[e];
-          s2 = fmaf(gv[e], xh, s2);
+          p1 += gv[e];
+          p2 = fmaf(gv[e], xh, p2);
         } else {
           gv[e] = rstd * (gv[e] - s1 - xh * s2);
           if (g.dres) gv[e] += res[e];
         }
       }
+      t1 += (double)p1;
+      t2 += (double)p2;
       if (pass) store8((TX*)g.dx + r * g.d, c, g.d, gv);
     }
     if (pass == 0) {
-      const float2 sum = row_sums<kWaves>(s1, s2, s_red, 0);
+      const float2 sum = row_sums<kWaves>((float)t1, (float)t2, s_red, 0);
       s1 = sum.x / (float)g.d;
       s2 = sum.y / (float)g.d;
     }
   }
 }
 
-// dw and db terms of rows gridDim.y apart, a column a thread.
+constexpr int kAnyRows = 4;  // rows that a lane below loads before the first is added
+
+// dw and db terms of those widths: a workgroup takes `cols` columns (a power of
+// two) by 256 / cols rows at once, rows gridDim.y times as many apart, in 64
+// bits as above. 2^24 rows x 4 in bfloat16: MEASURED
 template <typename TX, typename TY>
-__global__ __launch_bounds__(64 * kWaves) void norm_cols_any_kernel(const NormArgs g) {
-  const int64_t c = (int64_t)blockIdx.x * 64 * kWaves + threadIdx.x;
-  if (c >= g.d) return;
-  float aw = 0.f, ab = 0.f;
-  for (int64_t r = blockIdx.y; r < g.rows; r += gridDim.y) {
-    const float dy = (float)((const TY*)g.dy)[r * g.dy_ld + c];
-    aw = fmaf(dy, ((float)((const TX*)g.x)[r * g.x_ld + c] - g.mean[r]) * g.rstd[r], aw);
-    ab += dy;
+__global__ __launch_bounds__(64 * kWaves) void norm_cols_any_kernel(const NormArgs g, int cols) {
+  __shared__ double s_acc[2][64 * kWaves];
+  const int t = threadIdx.x, per = 64 * kWaves / cols;
+  const int64_t c = (int64_t)blockIdx.x * cols + (t & (cols - 1));
+  double aw = 0.0, ab = 0.0;
+  constexpr int kU = kAnyRows;  // added in float32 among themselves
+  const int64_t hop = (int64_t)gridDim.y * per;
+  if (c < g.d)
+    for (int64_t r0 = (int64_t)blockIdx.y * per + t / cols; r0 < g.rows; r0 += kU * hop) {
+      float dy[kU], xh[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int64_t r = r0 + u * hop < g.rows ? r0 + u * hop : r0;
+        dy[u] = (float)((const TY*)g.dy)[r * g.dy_ld + c];
+        xh[u] = ((float)((const TX*)g.x)[r * g.x_ld + c] - g.mean[r]) * g.rstd[r];
+      }
+      float pw = 0.f, pb = 0.f;
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (r0 + u * hop < g.rows) {
+          pw = fmaf(dy[u], xh[u], pw);
+          pb += dy[u];
+        }
+      aw += (double)pw;
+      ab += (double)pb;
+    }
+  // the rows' lanes join in halves
+  s_acc[0][t] = aw;
+  s_acc[1][t] = ab;
+  for (int h = per / 2; h >= 1; h >>= 1) {
+    __syncthreads();
+    if (t < h * cols) {
+      s_acc[0][t] += s_acc[0][t + h * cols];
+      s_acc[1][t] += s_acc[1][t + h * cols];
+    }
   }
-  float* part = g.part + (int64_t)blockIdx.y * 2 * g.d;
-  part[c] = aw;
-  part[g.d + c] = ab;
+  if (t < cols && c < g.d) {
+    float* part = g.part + (int64_t)blockIdx.y * 2 * g.d;
+    part[c] = (float)s_acc[0][t];
+    part[g.d + c] = (float)s_acc[1][t];
+  }
 }
 
-// dw[c], db[c] = the sums over n rows of part [n][2][d], in a fixed order: 32
-// columns a workgroup at a time, each of 32 groups of lanes adds every 32nd row.
+// dw[c], db[c] = the sums over n rows of part [n][2][d], in a fixed order and in
+// 64 bits (n grows with the rows): 32 columns a workgroup at a time, each of 32
+// groups of lanes adds every 32nd row.
 __global__ __launch_bounds__(1024) void norm_fold_kernel(const float* __restrict__ part, int n, int64_t d,
                                                          float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float s[32][33];
+  __shared__ double s[32][33];
   const int col = threadIdx.x & 31, q = threadIdx.x >> 5;
   for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < 2 * d; c0 += (int64_t)gridDim.x * 32) {
     const int64_t c = c0 + col;
-    float acc = 0.f;
+    double acc = 0.0;
     if (c < 2 * d) {
       constexpr int kU = 8;  // rows loaded before the first is added
       int i = q;
@@ -412,13 +456,13 @@ __global__ __launch_bounds__(1024) void norm_fold_kernel(const float* __restrict
     s[q][col] = acc;
     __syncthreads();
     if (q == 0 && c < 2 * d) {
-      float t = 0.f;
+      double t = 0.0;
 #pragma unroll
       for (int w = 0; w < 32; ++w) t += s[w][col];
       if (c < d) {
-        if (dw) dw[c] = t;
+        if (dw) dw[c] = (float)t;
       } else if (db) {
-        db[c - d] = t;
+        db[c - d] = (float)t;
       }
     }
     __syncthreads();
@@ -451,18 +495,27 @@ bool dt_ok(int dt) { return dt == NAJU_DTYPE_F32 || dt == NAJU_DTYPE_BF16 || dt 
 constexpr int64_t held(int wpr, int G) { return (int64_t)wpr * G * 64 * kV; }
 bool in_registers(int64_t d) { return d >= kV && d <= held(kWaves, 8); }
 
-// Workgroups of the backward in registers: rows are taken in turn by 768 of them
-// at most, three on a CU, which also bounds the sums that the fold adds (65536 x
-// 4096 bf16: 352 us; 369 with 512 of them, 422 with 1024, 377 with 2048; 16384 x
-// 768: 26 us; 28, 31 and 35).
-constexpr int kBwdGrid = 768;
+// Workgroups of the backward in registers: rows are taken in turn by 768 of them,
+// three on a CU (65536 x 4096 bf16: 352 us; 369 with 512 of them, 422 with 1024,
+// 377 with 2048; 16384 x 768: 26 us; 28, 31 and 35). With so many rows that a
+// wave's float32 sums of dw and db would have more than kChain terms, by the
+// next multiple of 768 that keeps to it: terms of one sign are then off by
+// kChain 2^-24 at most.
+constexpr int kBwdGrid = 768, kChain = 1024;
 int64_t bwd_grid(int64_t rows, int64_t d) {
   const int64_t per = d <= held(1, 2) ? kWaves : 1;
   const int64_t n = (rows + per - 1) / per;
-  return n < kBwdGrid ? n : kBwdGrid;
+  if (n <= kBwdGrid) return n;
+  return (n + kBwdGrid * kChain - 1) / (kBwdGrid * kChain) * kBwdGrid;
 }
-// Row slices of norm_cols_any_kernel.
-int64_t any_slices(int64_t rows) { return rows < 64 ? rows : 64; }
+// Columns that a workgroup of norm_cols_any_kernel takes, and its row slices:
+// narrow rows are one workgroup wide, so that it takes many slices to fill the CUs.
+int any_cols(int64_t d) { return d > 4 ? (d < kV ? kV : 64 * kWaves) : d > 2 ? 4 : (int)d; }
+int64_t any_slices(int64_t rows, int64_t d) {
+  const int64_t per = 64 * kWaves / any_cols(d) * kAnyRows, most = d < kV ? 1024 : 64;
+  const int64_t n = (rows + per - 1) / per;
+  return n < most ? n : most;
+}
 
 // Rows of one launch of a workgroup a row: a launch has fewer than 2^32 threads.
 constexpr int64_t kLaunchRows = 1 << 23;
@@ -518,9 +571,10 @@ void bwd_launch(const NormArgs& g, float* dw, float* db, hipStream_t st) {
       norm_dx_any_kernel<TX, TY><<<dim3((unsigned)p.rows), blk, 0, st>>>(p);
     }
     if (g.part) {
-      n = any_slices(g.rows);
+      const int cols = any_cols(g.d);
+      n = any_slices(g.rows, g.d);
       norm_cols_any_kernel<TX, TY>
-          <<<dim3((unsigned)((g.d + 64 * kWaves - 1) / (64 * kWaves)), (unsigned)n), blk, 0, st>>>(g);
+          <<<dim3((unsigned)((g.d + cols - 1) / cols), (unsigned)n), blk, 0, st>>>(g, cols);
     }
   } else if (g.d <= held(1, 1))
     norm_bwd_kernel<TX, TY, 1, 1><<<grid, blk, 0, st>>>(g);
@@ -612,7 +666,7 @@ int naju_layernorm_fwd(const void* x, int64_t x_ld, const float* w, const float*
 
 size_t naju_layernorm_workspace_bytes(int64_t n_rows, int64_t d) {
   if (n_rows < 0 || d < 1) return 0;
-  const int64_t n = in_registers(d) ? bwd_grid(n_rows, d) : any_slices(n_rows);
+  const int64_t n = in_registers(d) ? bwd_grid(n_rows, d) : any_slices(n_rows, d);
   return (size_t)(n * 2 * d) * sizeof(float) + 256;
 }
 
