@@ -437,8 +437,10 @@ class NajuLM(nn.Module):
         def head(h, tied):
             if compute_dtype(h) is not None:
                 return linear_cross_entropy(h, self.head.weight, targets, ignore_index, reduction, tied)
-            out = F.cross_entropy(self.head(h).flatten(0, -2).float(), targets.reshape(-1), ignore_index=ignore_index,
-                                  reduction=reduction)
+            logits = self.head(h).flatten(0, -2)
+            # 16-bit logits (CPU autocast) in float32, as the kernels form them
+            logits = logits.float() if logits.dtype in (torch.float16, torch.bfloat16) else logits
+            out = F.cross_entropy(logits, targets.reshape(-1), ignore_index=ignore_index, reduction=reduction)
             return out.view(targets.shape) if reduction == "none" else out
         return self._run(ids, head)
 
