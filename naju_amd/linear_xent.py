@@ -29,7 +29,7 @@ import torch
 from naju_amd import _lib, wcast
 from naju_amd.linear import compute_dtype
 
-_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
 class _ToTied(torch.autograd.Function):
@@ -56,8 +56,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean",
     must not be None; see the module's docstring. tied: a
     naju_amd.embed.TiedGrad that takes the weight's gradient for the tied
     embedding's backward, as in naju_amd.linear.lm_head."""
-    if reduction not in _REDUCTIONS:
-        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
     dt = compute_dtype(x)
     if dt is None or not x.is_floating_point():
         raise ValueError("naju_amd.linear_xent.linear_cross_entropy serves CUDA tensors computed in float16 / "
@@ -80,4 +80,4 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean",
     if tied is not None:
         weight = _ToTied.apply(weight, tied)
     return _lib.ops().linear_cross_entropy(x if x.dtype == dt else x.to(dt), weight, target, w16, int(ignore_index),
-                                           _REDUCTIONS[reduction])
+                                           REDUCTIONS[reduction])

@@ -42,7 +42,7 @@ from naju_amd.gated import ACTIVATIONS, gated_linear
 from naju_amd.layernorm import layer_norm, layer_norm_fork
 from naju_amd.layernorm import supported as layernorm_supported
 from naju_amd.linear import HEAD_ALIGN, compute_dtype, linear, linear_cat, lm_head
-from naju_amd.linear_xent import linear_cross_entropy
+from naju_amd.linear_xent import REDUCTIONS, linear_cross_entropy
 from naju_amd.optim import AdamW as NajuAdamW
 from naju_amd.readout import readout
 from naju_amd.rmsnorm import rms_norm
@@ -434,6 +434,14 @@ class NajuLM(nn.Module):
         """F.cross_entropy of forward(ids) against targets (ids' shape), the
         training loss of evals/lm/train.py:70-74; on CUDA in 16-bit compute
         without the logits (naju_amd.linear_xent)."""
+        if targets.shape != ids.shape:
+            raise ValueError(f"targets must be {tuple(ids.shape)}, got {tuple(targets.shape)}")
+        if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
+            raise TypeError(f"targets must hold class indices, got {targets.dtype}")
+        if reduction not in REDUCTIONS:
+            raise ValueError(f"reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
+        targets = targets.to(device=ids.device, dtype=torch.int64)
+
         def head(h, tied):
             if compute_dtype(h) is not None:
                 return linear_cross_entropy(h, self.head.weight, targets, ignore_index, reduction, tied)

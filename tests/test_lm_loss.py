@@ -49,3 +49,23 @@ def test_16_bit_logits_are_taken_in_float32():
         loss = m.loss(ids, y)
     assert logits.dtype == torch.bfloat16 and loss.dtype == torch.float32
     assert torch.equal(loss, F.cross_entropy(logits.float().view(-1, VOCAB), y.view(-1)))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_targets_have_the_ids_shape(device):
+    """The same targets are taken and refused on every path: ids' shape, class
+    indices of any integer type."""
+    m = _model() if device == "cpu" else NajuLM(VOCAB, d_model=16, n_layers=1, dropout=0.0, d_state=2).cuda()
+    ids, y = (t.to(device) for t in _batch())
+    for auto in (False, True):
+        with torch.autocast(device, dtype=torch.bfloat16, enabled=auto):
+            want = m.loss(ids, y)
+            assert torch.equal(m.loss(ids, y.int()), want)
+            for bad in (y.reshape(-1), y[:, :6], y.t(), y[None]):
+                with pytest.raises(ValueError, match="targets must be"):
+                    m.loss(ids, bad)
+            for bad in (y.float(), y == 3):
+                with pytest.raises(TypeError, match="class indices"):
+                    m.loss(ids, bad)
+            with pytest.raises(ValueError, match="reduction"):
+                m.loss(ids, y, reduction="median")
