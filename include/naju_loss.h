@@ -92,9 +92,16 @@ int naju_linear_xent_fwd(const void* x, int64_t x_ld, const void* w, int64_t w_l
                          void* stream);
 
 /* Bytes of workspace (256-byte aligned, no zero-fill) of the forward, or of
- * the backward when backward != 0: 1 GiB at most for the gradient of
- * a piece of the vocabulary's logits, n_rows * d float32, and the parts of
- * split products. */
+ * the backward when backward != 0. That holds
+ *   the 16-bit gradient of a piece of the vocabulary's logits: 1 GiB at most, or
+ *     512 bytes a row where that is more (above 2^21 rows: a piece has 256
+ *     columns at least);
+ *   x with the rows of ignored targets zero: 2 bytes for each of n_rows * d (d
+ *     rounded up to 8), and 4 bytes a row;
+ *   where the vocabulary takes several pieces, dx in float32: 4 n_rows d bytes;
+ *   the float32 parts of a product split over k, of one product at a time (none
+ *     where its result has many tiles): for d of 256 and more at most ten times,
+ *     below 64 times, the larger of dx and a piece's dw in float32. */
 size_t naju_linear_xent_workspace_bytes(int64_t n_rows, int64_t d, int64_t n_cols, int backward);
 
 /* Backward of naju_linear_xent_fwd, the logits formed again by pieces of the

@@ -235,8 +235,11 @@ int naju_gated_fwd(const void* x, int64_t x_ld, const void* w_gate, const void* 
                    int64_t h_ld, int64_t n_rows, int64_t d, int64_t f, int act, int dtype, void* stream);
 
 /* Bytes of workspace naju_gated_bwd needs (256-byte aligned, no zero-fill):
- * the projections' gradients in 16 bits, 4 n_rows f bytes, and the float32
- * parts of split products. */
+ * the projections' gradients in 16 bits, 4 bytes for each of n_rows * f (f
+ * rounded up to 32), and the float32 parts of a product split over k, of one
+ * product at a time (none where its result has many tiles): for d of 256 and
+ * more at most ten times, below 64 times, the larger of dx and both weights'
+ * gradients in float32. With few rows they are most of the workspace. */
 size_t naju_gated_workspace_bytes(int64_t n_rows, int64_t d, int64_t f);
 
 /* Backward of naju_gated_fwd from dh [n_rows, f] (dh_ld) in `dtype`, the

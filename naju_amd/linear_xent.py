@@ -9,9 +9,11 @@ evals/lm/train.py:70-74 in one, where naju_amd.linear.lm_head followed by
 naju_amd.xent.cross_entropy holds 16-bit logits and their gradient (3.3 GB at
 16384 tokens and 50257 classes). The logits stay in registers, float32 and
 unrounded; the forward keeps one float32 per row, and the backward forms them
-again by pieces of the vocabulary (1 GiB of workspace at most). It computes
-in x's 16-bit dtype, or in the autocast dtype under autocast (a weight of
-another dtype is cast, from naju_amd.wcast where it is active there).
+again by pieces of the vocabulary, in a workspace of at most 1 GiB (512 bytes
+a row above 2^21 rows) for a piece's gradient, 6 bytes for each element of x
+and the parts of split products. It computes in x's 16-bit dtype, or in the
+autocast dtype under autocast (a weight of another dtype is cast, from
+naju_amd.wcast where it is active there).
 
 The loss is float32: the mean over the rows whose target is not
 ignore_index ("mean"), their sum ("sum"), or a loss for every row with 0 for
