@@ -205,8 +205,8 @@ size_t naju_layernorm_workspace_bytes(int64_t n_rows, int64_t d);
 
 /* Backward of naju_layernorm_fwd: dx [n_rows, d] contiguous in x's dtype, and
  * dw, db [d] float32 (each nullable), summed over rows in a fixed order. dres
- * [n_rows, d] contiguous in x's dtype (nullable) is added to dx, as in
- * naju_rmsnorm_bwd_add. n_rows = 0 writes nothing. */
+ * [n_rows, d] contiguous in x's dtype (nullable; not dx itself) is added to
+ * dx, as in naju_rmsnorm_bwd_add. n_rows = 0 writes nothing. */
 int naju_layernorm_bwd(const void* x, int64_t x_ld, const float* w, const float* mean, const float* rstd,
                        const void* dy, int64_t dy_ld, const void* dres, void* dx, float* dw, float* db, int64_t n_rows,
                        int64_t d, int x_dtype, int dy_dtype, void* workspace, size_t workspace_bytes, void* stream);

@@ -20,9 +20,11 @@
 // What bounds it: 256 x 256 with eight waves of 128 x 64 reads 12 fragments of
 // 1 KB from LDS for 32 products, which keeps LDS (128 bytes a clock) and the
 // matrix cores about equally busy. Fragments of the next step are read behind
-// the products that used their registers last, with one barrier a step: 8192^3
-// in bf16 at 1290 TFLOP/s in any of the three layouts (1160 with two steps of
-// 64 k and the reads at the head of each; a library product here reaches 1440).
+// the products that used their registers last, with one barrier a step: 8192^3 in
+// bf16, random operands, at 1280 to 1340 TFLOP/s (least time of ten; 1140 to 1270 in
+// the mean, at 1.6 GHz) in any of the three layouts, matrix cores 63 to 73% busy, no
+// LDS bank conflicts (1160 with two steps of 64 k and the reads at the head of each,
+// when this loop stood at 1290; a library product reached 1440 then).
 // Four waves of 128 x 128 would read a third less, but the compiler moves
 // their accumulators between register files in the loop (110 TFLOP/s).
 //

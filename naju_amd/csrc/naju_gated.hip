@@ -157,9 +157,12 @@ __global__ __launch_bounds__(512) void gated_few_kernel(const GatedArgs g) {
 template <typename T, int ACT, bool BWD>
 void gated_launch(const GatedArgs& g, hipStream_t st) {
   // Few rows: bound by the latency of the weights' loads. Here and on the tiles
-  // below, d = 768 / 2048: 16 rows, f = 2048 4.6 / 9.0 and 11.5 / 26.6 us, f = 8192 7.9 /
-  // 16.5 and 12.4 / 29.3; 32 rows, f = 8192 9.3 / 20.3 and 12.7 / 29.5; 64 rows, f = 4096 8.2
-  // / 15.8 and 12.8 / 28.1, f = 5504 14.1 / 28.3 and 12.8 / 28.9.
+  // below, cold weights, d = 768 / 2048 / 8192: 16 rows, f = 1024 4.5 / 7.8 / 27.8 and
+  // 9.2 / 19.4 / 97.9 us, f = 8192 8.2 / 16.9 / 60.9 and 12.9 / 29.7 / 107, f = 28672 22.9 /
+  // 56.8 / 212 and 24.6 / 58.1 / 222, f = 65536 (768 / 2048) 47.4 / 124 and 49.1 / 132; 32
+  // rows, f = 8192 9.6 / 20.6 / 74.6 and 13.3 / 29.9 / 108, f = 16384 16.6 / 39.9 / 151 and
+  // 14.9 / 34.3 / 136; 64 rows, f = 4096 8.6 / 16.2 / 54.9 and 12.9 / 28.9 / 102, f = 5504
+  // 14.6 / 28.9 / 104 and 13.3 / 29.5 / 106.
   if (!BWD && (g.m <= 16 || (g.m <= 32 && g.f <= 8192) || (g.m <= 64 && g.f <= 4096))) {
     const unsigned grid = (unsigned)ceil_div(g.f, 16);
     if (g.m <= 16)
@@ -173,9 +176,14 @@ void gated_launch(const GatedArgs& g, hipStream_t st) {
   // backward tiles also cover the zero columns up to fp
   const int64_t f = BWD ? g.fp : g.f;
   const int64_t tl = ceil_div(g.m, TileL::BM) * ceil_div(f, TileL::BN / 2);
-  // the large tile where the small ones, two a CU, would need a second round
-  // (2048 rows, d = 768, forward: f = 2048, 128 large tiles, 19.8 us and 17.8 on
-  // small ones; f = 2560 20.7 and 23.6; f = 1024 18.8 and 10.7)
+  // the large tile where the small ones, two a CU, would need a second round. Both
+  // measured over 48 to 512 large tiles, d = 256, 768 and 2048 (2032 rows, d = 768;
+  // large and small): forward 96 tiles 20.0 and 16.0 us, 128 20.3 and 18.3, 144 20.5
+  // and 23.6, 256 26.3 and 38.1, 512 52.1 and 71.1; backward 128 27.8 and 23.8, 144
+  // 27.4 and 32.1, 256 31.6 and 41.0, 512 64.0 and 90.6. The rule loses where the
+  // large tiles have just begun a second round themselves, 257 to about 300 of them:
+  // at d = 768 up to 9% (288 tiles of 4080 rows backward 52.5 and 48.3), at d = 2048 up
+  // to 4%, at d = 256 up to 19%.
   if (tl > kCUs / 2) {
     const int nm = (int)ceil_div(g.m, TileL::BM), nn = (int)ceil_div(f, TileL::BN / 2);
     gated_kernel<T, TileL, ACT, BWD><<<tile_grid<TileL>(nm * nn), TileL::kThreads, 0, st>>>(g, nm, nn);

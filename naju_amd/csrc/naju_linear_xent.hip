@@ -372,16 +372,26 @@ __global__ __launch_bounds__(256) void head_mask_kernel(const uint16_t* __restri
 
 // ------------------------------------------------------------------ host side
 
-// The large tile where the small ones, two a CU, would need a second round (as
-// measured at the gated product's choice, naju_gated.hip).
+// The large tile where the small ones, two a CU, would need a second round. Both
+// measured over 48 to 512 large tiles, 240 to 16368 rows, d = 256, 768 and 2048
+// (1008 rows, d = 768; large and small): forward 96 tiles 24.5 and 20.1 us, 128 27.0
+// and 24.7, 144 27.9 and 33.8, 256 31.8 and 42.6, 512 56.8 and 75.4; gradient of the
+// logits 128 31.1 and 26.7, 144 31.2 and 33.3, 256 36.7 and 50.2, 512 66.2 and 95.4.
+// The rule loses where the large tiles have just begun a second round themselves,
+// 257 to about 300 of them: at d = 768 up to 11% (288 tiles of 4080 rows forward 46.7
+// and 42.7), at d = 2048 up to 6%, at d = 256 up to 17% forward and 29% for the
+// gradient, and to 384 tiles up to 14%; and at d = 256 from 129 to 176 tiles of the
+// gradient, up to 11%.
 bool head_large(int64_t m, int64_t v) { return ceil_div(m, TileL::BM) * ceil_div(v, TileL::BN) > kCUs / 2; }
 
-// Few rows: bound by the loads of W. With the join, here and on the tiles below, for
-// d = 768 / 2048: 1 row over 4096 classes 7.5 / 10.6 and 15.7 / 31.3 us, over 50257 19.5 /
-// 46.1 and 28.8 / 54.1; 16 rows 8.3 / 12.6 and 16.2 / 31.6, 25.2 / 57.3 and 28.8 / 54.2; 32
-// rows 9.6 / 14.8 and 16.4 / 31.8, 12347 classes 13.0 / 24.0 and 17.1 / 33.3, 50257 29.6 /
-// 68.1 and 29.0 / 54.4; 64 rows over 4096 11.4 / 18.9 and 16.8 / 32.3, 12347 18.5 / 33.4 and
-// 17.7 / 33.9. (A launch has fewer than 2^32 threads, 16 a column here.)
+// Few rows: bound by the loads of W. With the join, here and on the tiles below,
+// cold weights, d = 768 / 2048 / 4096: 1 row over 4096 classes 7.0 / 10.7 / 15.9 and
+// 12.6 / 31.6 / 56.6 us, over 50257 19.9 / 45.0 / 89.9 and 29.2 / 61.2 / 106; 16 rows
+// 8.1 / 13.0 / 19.7 and 12.9 / 32.0 / 56.9, 25.2 / 57.8 / 109 and 29.5 / 61.5 / 110, over
+// 131072 51.6 / 127 / 247 and 59.5 / 139 / 238 (the only loss to 16 rows, 4%); 32 rows
+// over 24576 17.3 / 35.8 / 64.1 and 18.8 / 36.3 / 63.3, 50257 29.8 / 68.5 / 132 and 30.1 /
+// 62.0 / 110; 64 rows over 4096 11.2 / 19.4 / 32.0 and 13.8 / 32.9 / 57.8, 12347 19.1 / 33.8
+// / 59.0 and 18.2 / 34.3 / 60.9. (A launch has fewer than 2^32 threads, 16 a column here.)
 bool head_few(int64_t m, int64_t v) {
   return (m <= 16 && v <= 1 << 27) || (m <= 32 && v <= 24576) || (m <= 64 && v <= 8192);
 }
