@@ -39,16 +39,18 @@ void loss_clear();
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.69314718055994531f;
 
-// (m, s): a maximum and the sum of 2^((v - m) log2 e) over a set; the empty
-// set is (-inf, 0). A NaN among the values or an infinite maximum gives a NaN
-// sum, as the softmax of such a row has.
-__device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
-__device__ __forceinline__ void ms_join(float& m, float& s, float m2, float s2) {
-  const float mn = fmaxf(m, m2), ref = ref_of(mn);
-  s = s * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * kLog2e);
-  m = mn;
+// (r, s) of a set of logits: r = max * log2 e, rounded, and the sum of
+// 2^(v log2 e - r); the empty set is (-inf, 0). Every exponent is formed against
+// that same r, so its rounding (2^-24 of a large maximum) is in the sum and in
+// the target's exponent alike and out of their difference, the row's loss. A NaN
+// among the values or an infinite maximum gives a NaN sum, as the softmax of
+// such a row has.
+__device__ __forceinline__ float ref_of(float r) { return r == -INFINITY ? 0.f : r; }
+__device__ __forceinline__ void ms_join(float& r, float& s, float r2, float s2) {
+  const float rn = fmaxf(r, r2), ref = ref_of(rn);
+  s = s * __builtin_amdgcn_exp2f(r - ref) + s2 * __builtin_amdgcn_exp2f(r2 - ref);
+  r = rn;
 }
 
 struct HeadArgs {
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void head_kernel(const HeadArgs g, 
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float ref = ref_of(mx) * kLog2e;
+        const float top = mx * kLog2e, ref = ref_of(top);
         float s = 0.f;
 #pragma unroll
         for (int j = 0; j < C::TN; ++j)
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void head_kernel(const HeadArgs g, 
           for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -ref));
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
-        if (lane < 16) s_ms[wn][mt + i * 16] = make_float2(mx, s);
+        if (lane < 16) s_ms[wn][mt + i * 16] = make_float2(top, s);
         if (m < g.m) {
           const int64_t target = g.target[m], t = target - nw;
           if (t >= 0 && t < 64 && target < g.v) {
@@ -206,20 +208,22 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(const HeadArgs g)
   static_assert(kSlices >= 4 && kSlices <= 64, "a row's lanes lie in one wave");
   const int m = threadIdx.x / kSlices, q = threadIdx.x % kSlices;
   const int64_t target = m < g.m ? g.target[m] : -1;
-  float mx = -INFINITY, sum = 0.f;
+  float r = -INFINITY, sum = 0.f;
   for (int n = q; n < P::N; n += kSlices)
     if (n0 + n < g.v) {
       const float v = s[n * P::M + m];
       if (n0 + n == target) g.at_target[m] = v;
-      // a value joins as its own set, so that a NaN reaches the sum
-      ms_join(mx, sum, fmaxf(v, -INFINITY), __builtin_amdgcn_exp2f((v - ref_of(fmaxf(v, -INFINITY))) * kLog2e));
+      // (fmaxf leaves a NaN out of r; it reaches the sum)
+      const float rn = fmaxf(r, fmaxf(v, -INFINITY) * kLog2e), ref = ref_of(rn);
+      sum = sum * __builtin_amdgcn_exp2f(r - ref) + __builtin_amdgcn_exp2f(fmaf(v, kLog2e, -ref));
+      r = rn;
     }
 #pragma unroll
   for (int h = kSlices / 2; h >= 1; h >>= 1) {
-    const float mx2 = __shfl_xor(mx, h, 64), sum2 = __shfl_xor(sum, h, 64);
-    ms_join(mx, sum, mx2, sum2);
+    const float r2 = __shfl_xor(r, h, 64), sum2 = __shfl_xor(sum, h, 64);
+    ms_join(r, sum, r2, sum2);
   }
-  if (q == 0 && m < g.m) g.part[(int64_t)m * gridDim.x + blockIdx.x] = make_float2(mx, sum);
+  if (q == 0 && m < g.m) g.part[(int64_t)m * gridDim.x + blockIdx.x] = make_float2(r, sum);
 }
 
 // Joins the tiles' pairs of a row: R rows a workgroup, 1024 / R lanes of it a
@@ -237,7 +241,7 @@ __global__ __launch_bounds__(1024) void head_join_kernel(const float2* __restric
   const int row = threadIdx.x % R, q = threadIdx.x / R;
   const int64_t m = (int64_t)blockIdx.x * R + row;
   const int64_t mc = m < rows ? m : rows - 1;
-  float mx = -INFINITY, s = 0.f;
+  float r = -INFINITY, s = 0.f;
   for (int t0 = q; t0 < tiles; t0 += 4 * kLanes) {
     float2 p[4];
 #pragma unroll
@@ -248,41 +252,44 @@ __global__ __launch_bounds__(1024) void head_join_kernel(const float2* __restric
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (t0 + u * kLanes < tiles) ms_join(mx, s, p[u].x, p[u].y);
+      if (t0 + u * kLanes < tiles) ms_join(r, s, p[u].x, p[u].y);
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   auto join_lanes = [&](int n) {
 #pragma unroll
     for (int h = n / 2; h >= 1; h >>= 1) {
-      const float mx2 = __shfl_xor(mx, h, 64), s2 = __shfl_xor(s, h, 64);
-      ms_join(mx, s, mx2, s2);
+      const float r2 = __shfl_xor(r, h, 64), s2 = __shfl_xor(s, h, 64);
+      ms_join(r, s, r2, s2);
     }
   };
   if constexpr (R == 1) {
     // the waves' pairs, then the first wave's lanes join those
     join_lanes(64);
-    if (lane == 0) s_ms[wave][0] = make_float2(mx, s);
+    if (lane == 0) s_ms[wave][0] = make_float2(r, s);
     __syncthreads();
     const float2 p = s_ms[lane & 15][0];
-    mx = p.x;
+    r = p.x;
     s = p.y;
     join_lanes(16);
   } else {
     // wave w joins the 64 pairs of row w
-    s_ms[q][row] = make_float2(mx, s);
+    s_ms[q][row] = make_float2(r, s);
     __syncthreads();
     const float2 p = s_ms[lane][wave];
-    mx = p.x;
+    r = p.x;
     s = p.y;
     join_lanes(64);
   }
   const int64_t mw = (int64_t)blockIdx.x * R + (R == 1 ? 0 : wave);
   if ((R == 1 ? threadIdx.x : lane) != 0 || mw >= rows) return;
-  const float l = ref_of(mx) + __builtin_amdgcn_logf(s) * kLn2;
-  lse[mw] = l;
+  const float ref = ref_of(r);
+  const double log2s = (double)__builtin_amdgcn_logf(s), scale = 1.0 / (double)kLog2e;
+  lse[mw] = (float)(((double)ref + log2s) * scale);
   const int64_t t = target[mw];
   // ignored rows are 0; a target outside the vocabulary is NaN
-  row_loss[mw] = t == ignore ? 0.f : (t >= 0 && t < cols ? l - at_target[mw] : __builtin_nanf(""));
+  row_loss[mw] = t == ignore ? 0.f
+                 : t >= 0 && t < cols ? (float)((log2s - (double)fmaf(at_target[mw], kLog2e, -ref)) * scale)
+                                      : __builtin_nanf("");
 }
 
 // loss = the rows' sum (in float64, in a fixed order) times scale, with
