@@ -170,20 +170,38 @@ __global__ __launch_bounds__(C::kThreads, 2) void head_kernel(const HeadArgs g, 
       for (int i = 0; i < C::TM; ++i) {
         const int64_t m = m0 + mt + i * 16;
         if (m >= g.m) continue;
-        const float c = g.coef[m], l2 = g.lse[m] * kLog2e;
+        const float c = g.coef[m], lse = g.lse[m];
         const int64_t t = g.target[m] - g.v0 - nw;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int64_t n = nw + h * 32;
           if (n >= g.dl_ld) continue;
           float o[8];
+          // (the difference first: it is exact near lse, and p of a row's one class 1)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(acc[i][2 * h + (e >> 2)][e & 3], kLog2e, -l2));
-            // an ignored row's gradient is 0 whatever its logits are
-            o[e] = n + e < g.v && c != 0.f ? c * (p - (t == h * 32 + e ? 1.f : 0.f)) : 0.f;
+          for (int e = 0; e < 8; ++e)
+            o[e] = __builtin_amdgcn_exp2f((acc[i][2 * h + (e >> 2)][e & 3] - lse) * kLog2e);
+          // few waves hold a target here, and only the last tiles columns past the end
+          const int64_t th = t - h * 32;
+          if (__ballot(th >= 0 && th < 8)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] -= th == e ? 1.f : 0.f;
           }
-          store_row((T*)g.dl + m * g.dl_ld + n, o, 8);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] *= c;
+          if (n0 + C::BN > g.v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = n + e < g.v ? o[e] : 0.f;
+          }
+          // an ignored row's gradient is 0 whatever its logits are
+          typedef typename UserVec<T, 8, sizeof(T)>::type vec;
+          typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+          vec v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = (T)o[e];
+          const u4 bits = __builtin_bit_cast(u4, v);
+          *reinterpret_cast<vec*>((T*)g.dl + m * g.dl_ld + n) =
+              __builtin_bit_cast(vec, c != 0.f ? bits : u4{0, 0, 0, 0});
         }
       }
     }

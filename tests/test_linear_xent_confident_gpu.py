@@ -31,3 +31,27 @@ def test_confident_rows(gpu, rows, v, scale):
     want = torch.log(torch.exp(gap).sum(1)) if float(gap.max()) < 600 else torch.logsumexp(gap, 1)
     got = linear_cross_entropy(x.to(gpu), w.to(gpu), t.to(gpu), reduction="none").double().cpu()
     assert ((got - want).abs() <= 2.0 ** -18 * (1 + want)).all(), float((got - want).abs().max())
+
+
+@pytest.mark.parametrize("rows, v", [(16, 300), (200, 700), (3000, 9000)])
+@pytest.mark.parametrize("scale", [3.0, 296.0])
+def test_gradient_of_rows_without_doubt(gpu, rows, v, scale):
+    """Where every other class is exp(-64) or less, dl is 0 up to float32's
+    rounding of p near 1 (2^-23), however large the logits (up to 2^15): dx and
+    dw, its products with entries of 1 and `scale`, are below 2^-21 of those."""
+    d = 128
+    g = torch.Generator().manual_seed(rows + v)
+    w = (torch.randint(0, 2, (v, d), generator=g) * 2 - 1).to(torch.bfloat16)
+    t = torch.randint(0, v, (rows,), generator=g)
+    x = (w[t] * scale).to(torch.bfloat16)
+    x[:, : 5] *= -1  # logits that no power of two divides
+    logits = x.double() @ w.double().t()
+    gap = logits - logits.gather(1, t[:, None])
+    gap[torch.arange(rows), t] = -1e9
+    keep = gap.max(1).values <= -64
+    assert keep.sum() > rows // 2
+    x, t = x[keep].to(gpu).requires_grad_(True), t[keep].to(gpu)
+    wr = w.to(gpu).requires_grad_(True)
+    dx, dw = torch.autograd.grad(linear_cross_entropy(x, wr, t, reduction="sum"), (x, wr))
+    assert float(dx.abs().max()) <= 2.0 ** -21
+    assert float(dw.abs().max()) <= 2.0 ** -21 * scale * float(torch.bincount(t).max())
