@@ -399,14 +399,13 @@ __global__ __launch_bounds__(256) void head_mask_kernel(const uint16_t* __restri
 
 // The large tile where the small ones, two a CU, would need a second round. Both
 // measured over 48 to 512 large tiles, 240 to 16368 rows, d = 256, 768 and 2048
-// (1008 rows, d = 768; large and small): forward 96 tiles 24.5 and 20.1 us, 128 27.0
-// and 24.7, 144 27.9 and 33.8, 256 31.8 and 42.6, 512 56.8 and 75.4; gradient of the
-// logits 128 31.1 and 26.7, 144 31.2 and 33.3, 256 36.7 and 50.2, 512 66.2 and 95.4.
+// (1008 rows, d = 768; large and small): forward 96 tiles 24.5 and 20.0 us, 128 27.1
+// and 24.7, 144 28.0 and 33.8, 256 31.3 and 42.8, 512 56.2 and 74.8; gradient of the
+// logits 128 29.5 and 26.0, 144 29.5 and 33.0, 256 35.1 and 51.6, 512 63.1 and 98.4.
 // The rule loses where the large tiles have just begun a second round themselves,
-// 257 to about 300 of them: at d = 768 up to 11% (288 tiles of 4080 rows forward 46.7
-// and 42.7), at d = 2048 up to 6%, at d = 256 up to 17% forward and 29% for the
-// gradient, and to 384 tiles up to 14%; and at d = 256 from 129 to 176 tiles of the
-// gradient, up to 11%.
+// 257 to about 300 of them: at d = 768 up to 11% (288 tiles of 4080 rows forward 46.3
+// and 42.2), at d = 2048 up to 5%, at d = 256 up to 17% forward and 21% for the
+// gradient, and 10% there from 301 to 512 tiles.
 bool head_large(int64_t m, int64_t v) { return ceil_div(m, TileL::BM) * ceil_div(v, TileL::BN) > kCUs / 2; }
 
 // Few rows: bound by the loads of W. With the join, here and on the tiles below,
