@@ -261,3 +261,49 @@ def test_in_place_changes_of_what_is_kept_are_noticed(gpu):
                 xi.add_(1)
             with pytest.raises(RuntimeError, match="inplace"):
                 loss.backward()
+
+
+@pytest.mark.gpu
+def test_inference_mode(gpu):
+    for d in (72, 71):
+        x, w, t = _inputs(d)
+        with torch.no_grad():
+            want = (layer_norm(x), *layer_norm_fork(x), gated_linear(x, w, w), linear_cross_entropy(x, w, t))
+        x.requires_grad_(True), w.requires_grad_(True)
+        with torch.inference_mode():
+            got = (layer_norm(x), *layer_norm_fork(x), gated_linear(x, w, w), linear_cross_entropy(x, w, t))
+            again = (layer_norm(x.clone()), *layer_norm_fork(x.clone()), gated_linear(x.clone(), w, w),
+                     linear_cross_entropy(x.clone(), w, t))
+        for a, b, c in zip(got, want, again):
+            assert torch.equal(a, b) and torch.equal(c, b)
+        # (the fork's stream is x's view, of which torch says what it says of x)
+        assert not any(a.requires_grad for i, a in enumerate(got) if i != 1)
+
+
+@pytest.mark.gpu
+def test_jit_trace_holds_the_operators(gpu):
+    x, w, t = _inputs(72)
+    with torch.no_grad():
+        g = torch.jit.trace(lambda x, w, t: (layer_norm(x), gated_linear(x, w, w), linear_cross_entropy(x, w, t)), (x, w, t))
+        x2 = x * 0.5
+        for a, b in zip(g(x2, w, t), (layer_norm(x2), gated_linear(x2, w, w), linear_cross_entropy(x2, w, t))):
+            assert torch.equal(a, b)
+    assert "naju::gated_linear" in str(g.graph)
+
+
+@pytest.mark.gpu
+def test_recomputed_and_selectively_kept_steps(gpu):
+    """Activation checkpointing, and its selective form, which keeps results by operator under a mode of its own."""
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+    keep = {torch.ops.naju._gated_fwd.default, torch.ops.naju._layer_norm_fwd.default}
+
+    def policy(ctx, op, *args, **kwargs):
+        return CheckpointPolicy.MUST_SAVE if op in keep else CheckpointPolicy.PREFER_RECOMPUTE
+
+    for d in (72, 71):
+        ins = _inputs(d)
+        want = _with_grads(_user_step, *ins)
+        for kw in ({}, {"context_fn": lambda: create_selective_checkpoint_contexts(policy)}):
+            got = _with_grads(lambda *a: checkpoint(_user_step, *a, use_reentrant=False, **kw), *ins)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
